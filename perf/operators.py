@@ -8,7 +8,6 @@ operations, ``own = True`` through polarflash_b200.  Sizes are this
 repository's: 32 query and 8 KV heads of 128 (or 64 query heads over 8), the
 small models' heads of 64, the vocabulary of 128256, and generic ones.
 """
-import functools
 import math
 import os
 import random
@@ -23,7 +22,6 @@ DTYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
 ROPE_THETA = 500000.0
 
 
-@functools.lru_cache(maxsize=None)
 def _api():
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "polar-flash_b200")
     if not os.path.isdir(root):

@@ -202,13 +202,17 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // (its bits taken from x + 1.5 2^23), 2^f for |f| <= 1/2 by the polynomial of
 // least relative error (degree 3: 7.5e-5, a fiftieth of bf16's half step;
 // degree 4: 2.6e-6, a two-hundredth of fp16's), n added to the exponent.
-// x >= -126 (-inf gives 2^-126), x <= 127; NaN gives a value that does not
-// stay finite.
+// x <= 127.  Masked and far lower scores end at kFloor, just above -127: there
+// n = -127 takes the exponent of a polynomial a little above 1 to zero, and what
+// is left, about 2^-139, is 0 in either type (2^-126 is a bf16 number, which a
+// large v would show).  Between kFloor and -126 the weight falls from 2^-126
+// to that.  NaN gives a value that does not stay finite.
+constexpr float kFloor = -126.9998f;
 template <typename T>
 __device__ __forceinline__ void ex2_poly(uint64_t x, float& lo, float& hi) {
   f2_split(x, lo, hi);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(kFloor));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(kFloor));
   x = f2(lo, hi);
   const uint64_t t = add2(x, f2(12582912.f, 12582912.f));
   const uint64_t f = fma2(add2(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);

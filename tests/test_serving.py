@@ -598,6 +598,36 @@ def test_prompt_attention_keeps_sequences_apart():
     assert (off <= (2.5 * 2.0 ** -8 + 0.1) * mag).all()
 
 
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_attention_weighs_hidden_keys_nothing(dt, hd):
+    """Values near the type's largest at keys that a row does not see, and at a
+    key whose score lies hundreds below the maximum, change nothing: their weight
+    is 0, in every place of a tile."""
+    P = _api()
+    g = _gen(hd)
+    n = 300
+    cu = _cu([n])
+    q, k, v = (torch.randn(n, h, hd, generator=g, device="cuda").to(dt) for h in (4, 2, 2))
+    big = torch.finfo(dt).max * 0.9
+    clean = P.prompt_attention(q, k, v, cu)
+    for first in (100, 128, 145, 200, 256, 272):
+        for j in range(16):
+            late = v.clone()
+            late[first + j::16] = big
+            got = P.prompt_attention(q, k, late, cu)
+            assert torch.equal(got[:first], clean[:first]), (first, j)
+    # one direction, along which key `at` scores 40 * 8 * sqrt(hd) / sqrt(hd) = 320 and more below every other
+    q = torch.full((n, 4, hd), 8.0, dtype=dt, device="cuda")
+    for at in (0, 1, 2, 17, 130, 144):
+        low = torch.randn(n, 2, hd, generator=g, device="cuda").to(dt).abs()
+        low[at] = -40.0
+        v0, v1 = v.clone(), v.clone()
+        v0[at], v1[at] = 0.0, big
+        assert torch.equal(P.prompt_attention(q, low, v1, cu)[at + 1:], P.prompt_attention(q, low, v0, cu)[at + 1:]), at
+
+
 # ---- the draw ---------------------------------------------------------------------
 def _draw64(logits, u, t, k, p, m):
     """One row, in Python's and torch's fp64, entry by entry."""

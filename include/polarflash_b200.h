@@ -463,6 +463,15 @@ PF_API int pf_prompt_attention(const void* q, long long q_stride, const void* k,
                                long long v_stride, void* out, long long out_stride, int dtype, const int* cu_q,
                                const int* cu_k, int seqs, int total_q, int total_k, int n_heads, int n_kv_heads,
                                int head_dim, float scale, int* status, void* stream);
+/* pf_prompt_attention with waits that give up after wait_ns (0 to 2e9) instead
+ * of two seconds: 0 gives up wherever a warp has to wait at all.  Rows of out
+ * are what pf_prompt_attention gives or, where their block gave up, NaN; status
+ * receives PF_ERR_TIMEOUT then.  A diagnostic of the give-up path for tests and
+ * deployment checks, as pf_wait_selftest. */
+PF_API int pf_prompt_selftest(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                              long long v_stride, void* out, long long out_stride, int dtype, const int* cu_q,
+                              const int* cu_k, int seqs, int total_q, int total_k, int n_heads, int n_kv_heads,
+                              int head_dim, float scale, int* status, unsigned long long wait_ns, void* stream);
 
 /* Draws one token per row of logits [rows][vocab] (rows row_stride elements
  * apart, `dtype`) with a given uniform number u[row] in [0, 1).  With w_i =

@@ -39,9 +39,12 @@
 // instead of one (527 against 516).  In bursts, against 443 us: steps of 64 keys
 // with two S buffers (558: 64-wide score products wait for Q's reads from shared
 // memory), a warp of products per tile (534: their products interleave).
-// Every wait is bounded; one that gives up marks the status word, the CTA's
-// rows become NaN, copies and products in flight are waited for, TMEM is
-// freed.
+// Every wait is bounded.  One that gives up raises the CTA's abort flag, on
+// which the other waits give up too; the status word is marked, and rows that
+// were still waiting become NaN.  The warps then meet at a barrier, and only
+// behind it, where nothing more is issued, the loading thread waits for every
+// copy that it issued and the issuing thread for its products, before TMEM is
+// freed and the block ends.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
@@ -73,6 +76,8 @@ struct PromptArgs {
   int seqs, total_q, total_k, G, nkv, hd;
   float scale_log2;
   unsigned* status;
+  unsigned poll_mask;          // of polls of a wait, those that look at the clock: every poll_mask + 1st
+  unsigned long long wait_ns;  // after which a wait gives up
 };
 
 template <int HD>
@@ -86,8 +91,11 @@ struct Cfg {
 // Bounded wait on an mbarrier phase, polling without a suspend hint and
 // looking at the clock and the abort flag every 64th time only (both cost
 // more than a poll, and the kernel's chain of waits is its critical path);
-// false when it gave up or another warp of the CTA did.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const volatile int* abort_flag) {
+// false when it gave up or another warp of the CTA did.  The answer is the
+// calling thread's own: a warp that goes on together takes a vote of it.
+constexpr unsigned kPollMask = 63;
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const volatile int* abort_flag, unsigned mask,
+                                         unsigned long long limit_ns) {
   unsigned long long t0 = 0;
   for (unsigned spin = 1;; ++spin) {
     uint32_t done;
@@ -97,12 +105,12 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const vo
         : "r"(bar), "r"(parity)
         : "memory");
     if (done) return true;
-    if (spin & 63) continue;
+    if (spin & mask) continue;
     if (*abort_flag) return false;
     const unsigned long long t = now_ns();
     if (t0 == 0)
       t0 = t;
-    else if (t - t0 > kWaitNs)
+    else if (t - t0 >= limit_ns)
       return false;
   }
 }
@@ -343,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ uint64_t bars[2 * kStages + 10];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  __shared__ int copies;  // ring entries whose copies were issued
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = smem_u32(&bars[0]), free0 = smem_u32(&bars[kStages]), qbar = smem_u32(&bars[2 * kStages]);
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const volatile int* abort_p = &abort_flag;
 
   if (threadIdx.x == 0) {
-    abort_flag = 0;
+    abort_flag = copies = 0;
     for (int s = 0; s < 2 * kStages + 10; ++s) {
       // p: the four softmax warps of a tile arrive
       const bool p = s >= 2 * kStages + 6;
@@ -370,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = tmem_slot;
   pdl_enter();
+  auto wait = [&](uint32_t bar, uint32_t parity) { return bar_wait(bar, parity, abort_p, a.poll_mask, a.wait_ns); };
   Job job;
   if (find_job(a, blockIdx.x, job)) {
     const int most = max(job.tiles[0], job.tiles[1]);
@@ -380,7 +390,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (warp == kTmaWarp) {
         // ---------------------------------------------------------- loads
         if (lane == 0 && most > 0) {
-          int issued = 0;
           const uint32_t nq = (job.tiles[0] > 0) + (job.tiles[1] > 0);
           mbar_expect(qbar, nq * C::kTileBytes);
 #pragma unroll
@@ -390,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tma_3d(base + t * C::kTileBytes + x * kBox, &qmap, 64 * x, job.head[t], job.q0 + job.row0[t], qbar);
           for (int i = 0; i < 2 * most; ++i) {  // K and V in turn
             const int slot = i % kStages;
-            if (i >= kStages && !bar_wait(free0 + 8 * slot, (i / kStages - 1) & 1, abort_p)) {
+            if (i >= kStages && !wait(free0 + 8 * slot, (i / kStages - 1) & 1)) {
               abort_flag = 1;
               break;
             }
@@ -398,95 +407,88 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_expect(bar, C::kTileBytes);
             for (int x = 0; x < C::kBoxes; ++x)
               tma_3d(dst + x * kBox, i & 1 ? &vmap : &kmap, 64 * x, job.kvh, job.k0 + (i >> 1) * kTile, bar);
-            issued = i + 1;
-          }
-          if (*abort_p) {  // copies in flight land before the block ends
-            const int never = 0;
-            bar_wait(qbar, 0, &never);
-            for (int i = max(0, issued - kStages); i < issued; ++i)
-              bar_wait(full0 + 8 * (i % kStages), (i / kStages) & 1, &never);
+            copies = i + 1;
           }
         }
       } else if (warp == kMmaWarp) {
         // ---------------------------------------------------------- products
         const uint32_t id_s = idesc(kBf16, kTile, false), id_o = idesc(kBf16, HD, true);
         auto score = [&](int t, int i) {  // S_t = Q_t K^T, K in ring entry i
-          if (elect_one()) {
-            const uint32_t sa = base + t * C::kTileBytes, sb = ring + (i % kStages) * C::kTileBytes;
+          const uint32_t sa = base + t * C::kTileBytes, sb = ring + (i % kStages) * C::kTileBytes;
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) {
-              const uint32_t off = (k >> 2) * kBox + (k & 3) * 32;
-              mma_ss(tmem + kTmemS + t * kTile, desc_k(sa + off), desc_k(sb + off), id_s, k > 0);
-            }
-            commit(sbar + 8 * t);
+          for (int k = 0; k < HD / 16; ++k) {
+            const uint32_t off = (k >> 2) * kBox + (k & 3) * 32;
+            mma_ss(tmem + kTmemS + t * kTile, desc_k(sa + off), desc_k(sb + off), id_s, k > 0);
           }
-          __syncwarp();
+          commit(sbar + 8 * t);
         };
-        bool ok = most > 0;
-        if (ok) ok = bar_wait(qbar, 0, abort_p) && bar_wait(full0, 0, abort_p);
-        if (ok) {
-          fence_after();
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (job.tiles[t] > 0) score(t, 0);
-          if (elect_one()) commit(free0);
-          __syncwarp();
-        }
-        for (int j = 0; ok && j < most; ++j) {
-          const int iv = 2 * j + 1, ik = 2 * j + 2;
-          ok = bar_wait(full0 + 8 * (iv % kStages), (iv / kStages) & 1, abort_p);
-          if (!ok) break;
-          const uint32_t sv = ring + (iv % kStages) * C::kTileBytes;
-          const int left = job.m - j * kTile;  // keys of the sequence in this tile
+        // The steps of one thread: it waits and issues by itself (a vote of the warp at each wait took 3 % of the
+        // kernel).  The warp meets before the last step, where a V tile that the sequence does not fill needs
+        // zeros, and once more at the end; `ok` is the same in all lanes there.
+        bool ok = true;
+        for (int from = 0; ok && from < most;) {
+          const int whole = job.m / kTile, to = from < whole && whole < most ? whole : most;
+          const int last = 2 * to - 1, left = job.m - (to - 1) * kTile;  // V of the last step, keys of the sequence in it
           if (left < kTile) {
+            const uint32_t sv = ring + (last % kStages) * C::kTileBytes;
+            ok = __all_sync(0xffffffffu, wait(full0 + 8 * (last % kStages), (last / kStages) & 1));
+            if (!ok) break;
             for (int r = left * 8 + lane; r < kTile * 8; r += 32)
               for (int x = 0; x < C::kBoxes; ++x)
                 asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + x * kBox + r * 16), "r"(0) : "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
           }
-          bool have_k = false;
+          if (elect_one()) {
+            if (from == 0) {
+              ok = wait(qbar, 0) && wait(full0, 0);
+              if (ok) {
+                fence_after();
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!ok || j >= job.tiles[t]) continue;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {  // P and the products with it in two halves of the keys
-              ok = ok && bar_wait(pbar + 16 * t + 8 * h, j & 1, abort_p);
-              if (!ok) continue;
-              fence_after();
-              if (elect_one()) {
-#pragma unroll
-                for (int k = 4 * h; k < 4 * h + 4; ++k)
-                  mma_ts(tmem + kTmemO + t * HD, tmem + kTmemS + t * kTile + 8 * k, desc_mn(sv + k * 2048), id_o,
-                         j > 0 || k > 0);
-                if (h) commit(obar + 8 * t);
+                for (int t = 0; t < 2; ++t)
+                  if (job.tiles[t] > 0) score(t, 0);
+                commit(free0);
               }
-              __syncwarp();
             }
-            if (!ok) continue;
-            if (j + 1 < job.tiles[t]) {
-              if (!have_k) ok = bar_wait(full0 + 8 * (ik % kStages), (ik / kStages) & 1, abort_p);
-              if (!ok) continue;
-              have_k = true;
-              fence_after();
-              score(t, ik);
+            for (int j = from; ok && j < to; ++j) {
+              const int iv = 2 * j + 1, ik = 2 * j + 2;
+              ok = wait(full0 + 8 * (iv % kStages), (iv / kStages) & 1);
+              if (!ok) break;
+              const uint32_t sv = ring + (iv % kStages) * C::kTileBytes;
+              bool have_k = false;
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                if (!ok || j >= job.tiles[t]) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // P and the products with it in two halves of the keys
+                  ok = ok && wait(pbar + 16 * t + 8 * h, j & 1);
+                  if (!ok) continue;
+                  fence_after();
+#pragma unroll
+                  for (int k = 4 * h; k < 4 * h + 4; ++k)
+                    mma_ts(tmem + kTmemO + t * HD, tmem + kTmemS + t * kTile + 8 * k, desc_mn(sv + k * 2048), id_o,
+                           j > 0 || k > 0);
+                  if (h) commit(obar + 8 * t);
+                }
+                if (!ok) continue;
+                if (j + 1 < job.tiles[t]) {
+                  if (!have_k) ok = wait(full0 + 8 * (ik % kStages), (ik / kStages) & 1);
+                  if (!ok) continue;
+                  have_k = true;
+                  fence_after();
+                  score(t, ik);
+                }
+              }
+              if (ok) {
+                commit(free0 + 8 * (iv % kStages));
+                if (j + 1 < most) commit(free0 + 8 * (ik % kStages));
+              }
             }
           }
-          if (ok && elect_one()) {
-            commit(free0 + 8 * (iv % kStages));
-            if (j + 1 < most) commit(free0 + 8 * (ik % kStages));
-          }
-          __syncwarp();
+          ok = __all_sync(0xffffffffu, ok);
+          from = to;
         }
-        if (most > 0 && !ok) {
-          abort_flag = 1;
-          const int never = 0;
-          if (lane == 0) {
-            commit(dbar);
-            bar_wait(dbar, 0, &never);
-          }
-          __syncwarp();
-        }
+        if (!ok) abort_flag = 1;
       }
     } else {
       // ---------------------------------------------------------- softmax
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < tiles; ++j) {
-        ok = __all_sync(0xffffffffu, bar_wait(sbar + 8 * t, j & 1, abort_p));
+        ok = __all_sync(0xffffffffu, wait(sbar + 8 * t, j & 1));
         if (!ok) break;
         fence_after();
         uint32_t v[kTile];
@@ -525,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mx = fmaxf(mx, m);
         const bool move = (mx - m) * c > kSlack;  // (also from -inf; false for NaN)
         if (__any_sync(0xffffffffu, move) && j > 0) {
-          ok = __all_sync(0xffffffffu, bar_wait(obar + 8 * t, (j - 1) & 1, abort_p));
+          ok = __all_sync(0xffffffffu, wait(obar + 8 * t, (j - 1) & 1));
           if (!ok) break;
           fence_after();
           const float f = !move ? 1.f : m == -INFINITY ? 0.f : ex2((m - mx) * c);
@@ -573,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         f2_split(add2(sum[0], sum[1]), x, y);
         l += x + y;
       }
-      if (ok && tiles > 0) ok = __all_sync(0xffffffffu, bar_wait(obar + 8 * t, (tiles - 1) & 1, abort_p));
+      if (ok && tiles > 0) ok = __all_sync(0xffffffffu, wait(obar + 8 * t, (tiles - 1) & 1));
       if (!ok) {
         abort_flag = 1;
         if (lane == 0 && a.status) atomicExch(a.status, (unsigned)PF_ERR_TIMEOUT);
@@ -626,6 +628,23 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   fence_before();
   __syncthreads();
+  if (abort_flag) {  // block-uniform: raised before the barrier only
+    const int never = 0;
+    auto drain = [&](uint32_t bar, uint32_t parity) { bar_wait(bar, parity, &never, kPollMask, kWaitNs); };
+    if (threadIdx.x == 32 * kTmaWarp && copies > 0) {  // (Q goes out in front of the first of them)
+      drain(qbar, 0);
+      for (int i = max(0, copies - kStages); i < copies; ++i) drain(full0 + 8 * (i % kStages), (i / kStages) & 1);
+    }
+    if (warp == kMmaWarp) {
+      if (elect_one()) {  // the thread that issued the products: a commit covers its own
+        commit(dbar);
+        drain(dbar, 0);
+      }
+      __syncwarp();
+    }
+    fence_before();
+    __syncthreads();
+  }
   if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
@@ -671,10 +690,11 @@ cudaError_t launch_prompt(const CUtensorMap& q, const CUtensorMap& k, const CUte
 
 using namespace pfb;
 
-int pf_prompt_attention(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
-                        long long v_stride, void* out, long long out_stride, int dtype, const int* cu_q,
-                        const int* cu_k, int seqs, int total_q, int total_k, int n_heads, int n_kv_heads,
-                        int head_dim, float scale, int* status, void* stream) {
+static int prompt_attention(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                            long long v_stride, void* out, long long out_stride, int dtype, const int* cu_q,
+                            const int* cu_k, int seqs, int total_q, int total_k, int n_heads, int n_kv_heads,
+                            int head_dim, float scale, int* status, unsigned poll_mask, unsigned long long wait_ns,
+                            void* stream) {
   if (!q || !out || out == q || out == k || out == v || !cu_q || !cu_k || seqs < 0 || total_q < 0 || total_k < 0 || (total_k > 0 && (!k || !v)) ||
       !(scale > 0.f && scale <= 3e38f) || (dtype != PF_DTYPE_F16 && dtype != PF_DTYPE_BF16))
     return PF_ERR_INVALID_ARGUMENT;
@@ -703,11 +723,28 @@ int pf_prompt_attention(const void* q, long long q_stride, const void* k, long l
                 total_k ? v_stride : q_stride))
     return report_cuda(cudaErrorInvalidValue);
   const PromptArgs a{q, k, v, out, q_stride, k_stride, v_stride, out_stride, cu_q, cu_k, seqs, total_q, total_k, (int)G, n_kv_heads, head_dim,
-                     scale * 1.4426950408889634f, reinterpret_cast<unsigned*>(status)};
+                     scale * 1.4426950408889634f, reinterpret_cast<unsigned*>(status), poll_mask, wait_ns};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const unsigned n = (unsigned)blocks;
   const cudaError_t e =
       head_dim > 64 ? (bf16 ? launch_prompt<128, __nv_bfloat16>(qm, km, vm, a, n, s) : launch_prompt<128, __half>(qm, km, vm, a, n, s))
                     : (bf16 ? launch_prompt<64, __nv_bfloat16>(qm, km, vm, a, n, s) : launch_prompt<64, __half>(qm, km, vm, a, n, s));
   return e == cudaSuccess ? PF_OK : report_cuda(e);
+}
+
+int pf_prompt_attention(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                        long long v_stride, void* out, long long out_stride, int dtype, const int* cu_q,
+                        const int* cu_k, int seqs, int total_q, int total_k, int n_heads, int n_kv_heads,
+                        int head_dim, float scale, int* status, void* stream) {
+  return prompt_attention(q, q_stride, k, k_stride, v, v_stride, out, out_stride, dtype, cu_q, cu_k, seqs, total_q,
+                          total_k, n_heads, n_kv_heads, head_dim, scale, status, kPollMask, kWaitNs, stream);
+}
+
+int pf_prompt_selftest(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
+                       long long v_stride, void* out, long long out_stride, int dtype, const int* cu_q,
+                       const int* cu_k, int seqs, int total_q, int total_k, int n_heads, int n_kv_heads, int head_dim,
+                       float scale, int* status, unsigned long long wait_ns, void* stream) {
+  if (wait_ns > kWaitNs) return PF_ERR_INVALID_ARGUMENT;
+  return prompt_attention(q, q_stride, k, k_stride, v, v_stride, out, out_stride, dtype, cu_q, cu_k, seqs, total_q,
+                          total_k, n_heads, n_kv_heads, head_dim, scale, status, 0, wait_ns, stream);
 }

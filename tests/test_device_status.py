@@ -74,3 +74,42 @@ def test_engine_check_raises_runtime_error():
     assert_rel(y.cpu().numpy(), oracle.linear("int2_g128", pay, 256, 1024, META, x.float().numpy()))
     check_device_status(dev, s)
     assert np.isfinite(y.cpu().numpy()).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("wait_ns", [0, 2000, 20000])
+def test_prompt_attention_that_gives_up_leaves_nothing_behind(hd, wait_ns):
+    """Waits of the prompt kernel that give up at once, or in the middle: the
+    status word says so, every row is right or NaN, and the blocks that come
+    behind on the same multiprocessors, whose shared memory a copy still in
+    flight would have overwritten, and later calls give what they give alone."""
+    from polarflash_b200 import _lib, prompt_attention
+
+    g = torch.Generator(device="cuda").manual_seed(hd)
+    lens = [700, 90, 1, 1500, 300] * 4
+    cu = torch.tensor([0] + lens, device="cuda").cumsum(0).to(torch.int32)
+    q, k, v = (torch.randn(sum(lens), h, hd, generator=g, device="cuda").bfloat16() for h in (8, 2, 2))
+    want = prompt_attention(q, k, v, cu)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    T, p = sum(lens), lambda t: ctypes.c_void_p(t.data_ptr())  # noqa: E731
+
+    def limited(out, limit):
+        s = torch.cuda.current_stream()
+        return _lib.load().pf_prompt_selftest(p(q), 8 * hd, p(k), 2 * hd, p(v), 2 * hd, p(out), 8 * hd, 2, p(cu), p(cu),
+                                              len(lens), T, T, 8, 2, hd, hd ** -0.5, p(status), limit, ctypes.c_void_p(s.cuda_stream))
+
+    out = torch.zeros_like(q)
+    assert limited(out, 2_000_000_001) == _lib.ERR_INVALID_ARGUMENT
+    for _ in range(3):
+        _lib.check(limited(out, wait_ns), "pf_prompt_selftest")
+        after = prompt_attention(q, k, v, cu)
+        assert torch.equal(after, want)
+        gone = out.isnan().all(-1)  # a row of a head is given up as a whole
+        assert (gone == out.isnan().any(-1)).all()
+        assert torch.equal(out[~gone], want[~gone])
+        assert int(status) == (_lib.ERR_TIMEOUT if gone.any() else _lib.OK)
+        if wait_ns == 0:
+            assert gone.any()
+        status.zero_()
+    _lib.check(limited(out, 2_000_000_000), "pf_prompt_selftest")
+    assert torch.equal(out, want) and int(status) == _lib.OK

@@ -214,7 +214,8 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // n = -127 takes the exponent of a polynomial a little above 1 to zero, and what
 // is left, about 2^-139, is 0 in either type (2^-126 is a bf16 number, which a
 // large v would show).  Between kFloor and -126 the weight falls from 2^-126
-// to that.  NaN gives a value that does not stay finite.
+// to that.  NaN gives a number near fp32's largest or more, which the row's sum
+// is looked at for.
 constexpr float kFloor = -126.9998f;
 template <typename T>
 __device__ __forceinline__ void ex2_poly(uint64_t x, float& lo, float& hi) {
@@ -574,6 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         float x, y;
         f2_split(add2(sum[0], sum[1]), x, y);
         l += x + y;
+        if (!(x + y <= 3.4e38f)) l = __int_as_float(0x7fffffff);  // a NaN that the polynomial made a number of
       }
       if (ok && tiles > 0) ok = __all_sync(0xffffffffu, wait(obar + 8 * t, (tiles - 1) & 1));
       if (!ok) {

@@ -628,6 +628,26 @@ def test_prompt_attention_weighs_hidden_keys_nothing(dt, hd):
         assert torch.equal(P.prompt_attention(q, low, v1, cu)[at + 1:], P.prompt_attention(q, low, v0, cu)[at + 1:]), at
 
 
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_attention_hands_nan_on(dt, hd):
+    """A NaN in k makes NaN of every value of the rows that see it, wherever in a
+    tile it stands and whatever scores follow it, and of no other row."""
+    P = _api()
+    n = 300
+    cu = _cu([n])
+    q, k, v = (torch.randn(n, h, hd, generator=_gen(hd), device="cuda").to(dt) for h in (4, 2, 2))
+    k[256:] *= 30  # larger scores later: what was summed up before is scaled down
+    clean = P.prompt_attention(q, k, v, cu)
+    for at in (*range(17), 128, 129, 145, 270):
+        bad = k.clone()
+        bad[at, 1, hd // 2] = math.nan
+        got = P.prompt_attention(q, bad, v, cu)
+        assert got[at:, 2:].isnan().all(), at
+        assert torch.equal(got[:at], clean[:at]) and torch.equal(got[:, :2], clean[:, :2])
+
+
 # ---- the draw ---------------------------------------------------------------------
 def _draw64(logits, u, t, k, p, m):
     """One row, in Python's and torch's fp64, entry by entry."""

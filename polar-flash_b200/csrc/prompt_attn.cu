@@ -585,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       fence_after();
       T* out = static_cast<T*>(a.out) + (long long)(job.q0 + row) * a.os + (long long)head * a.hd;
       const bool mine = head >= 0 && row < job.n;
-      const bool none = ok && m == -INFINITY && l < 1.f;  // no key seen
+      const bool none = ok && seen < 0;  // no key seen: zeros (and 0 / 0 where every score is -inf)
       const float inv = ok ? 1.f / l : __int_as_float(0x7fffffff);
 #pragma unroll
       for (int i = 0; i < HD; i += 32) {

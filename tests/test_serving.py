@@ -648,6 +648,33 @@ def test_prompt_attention_hands_nan_on(dt, hd):
         assert torch.equal(got[:at], clean[:at]) and torch.equal(got[:, :2], clean[:, :2])
 
 
+@gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_prompt_attention_of_infinite_scores(dt):
+    """Scores of -inf weigh nothing beside finite ones, before and behind them; a
+    row with nothing else is 0 / 0, NaN, as the definition has it, while a row
+    without keys is zeros."""
+    P = _api()
+    g = _gen(2)
+    n, hd = 200, 64
+    cu = _cu([n])
+    q = torch.rand(n, 2, hd, generator=g, device="cuda").to(dt) + 0.1
+    k, v = (torch.randn(n, 1, hd, generator=g, device="cuda").to(dt) for _ in range(2))
+    for cut in (1, 17, 128, 150):
+        low = k.clone()
+        low[:cut] = -math.inf
+        got = P.prompt_attention(q, low, v, cu)
+        assert got[:cut].isnan().all(), cut
+        # the same rows over the other keys alone
+        rest = P.prompt_attention(q[cut:], k[cut:], v[cut:], _cu([n - cut]))
+        e = HALF_STEP[dt]
+        _, mag = _prompt64(q[cut:], k[cut:], v[cut:], [0, n - cut], [0, n - cut], hd ** -0.5)
+        # each of the two is off by no more than the bound of a prompt
+        assert ((got[cut:].double() - rest.double()).abs() <= 2 * ((2.5 * e + 1.6e-5) * mag + 2.0 ** -24 * n)).all(), cut
+    few = P.prompt_attention(q[:20], low[:10], v[:10], _cu([20]), _cu([10]))
+    assert (few[:10] == 0).all() and few[10:].isnan().all()
+
+
 # ---- the draw ---------------------------------------------------------------------
 def _draw64(logits, u, t, k, p, m):
     """One row, in Python's and torch's fp64, entry by entry."""

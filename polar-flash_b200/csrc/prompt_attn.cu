@@ -4,7 +4,9 @@
 //   p = 2^(c (s - m)),  c = scale log2 e,   l += sum p,   O += P V,
 // where m only moves (and O and l are scaled by 2^(c (m_old - m_new))) when
 // the row's maximum has grown by more than 2^8: until then p <= 2^8, which
-// fp16 and bf16 hold as well as p <= 1, and the final O / l is the same.
+// fp16 and bf16 hold as well as p <= 1, and the final O / l is the same.  For
+// bf16, whose v may be near fp32's largest value, all p are lower by 2^20, so
+// that sums over a million keys of it stay finite.
 //
 // The 128-row query tiles of one (sequence, KV head) are numbered
 // x = (place in the prompt) * G + (query head in its group of G), and a CTA
@@ -66,6 +68,8 @@ constexpr int kTmaWarp = 8, kMmaWarp = 9;
 constexpr uint32_t kBox = kTile * 128;  // bytes of a 64-column box
 constexpr int kTmemS = 0, kTmemO = 256, kTmemCols = 512;
 constexpr float kSlack = 8.f;  // log2 of the largest p
+template <typename T>
+constexpr float kLower = std::is_same<T, __nv_bfloat16>::value ? 20.f : 0.f;  // p is 2^-kLower times the weight
 constexpr int kPoly = 1;       // of eight pairs of exponentials, those on the FMA pipes
 
 struct PromptArgs {
@@ -544,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (move) m = mx;
-        const float mc = m == -INFINITY ? 0.f : m * c;
+        const float mc = (m == -INFINITY ? 0.f : m * c) + kLower<T>;
         const uint64_t c2 = f2(c, c), mc2 = f2(-mc, -mc);
         uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
@@ -611,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // (a sum of weights that is not finite is the row's own: a score it sees is not)
           if ((nan || big > 3.4e38f) && ok && l <= 3.4e38f &&
               without_hidden<T>(a, job.q0 + row, head, job.k0, job.kvh, seen, min(job.m, tiles * kTile), i,
-                                m == -INFINITY ? 0.f : m * c, inv))
+                                (m == -INFINITY ? 0.f : m * c) + kLower<T>, inv))
             continue;
 #pragma unroll
           for (int e = 0; e < 32; e += 8)

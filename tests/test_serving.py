@@ -675,6 +675,27 @@ def test_prompt_attention_of_infinite_scores(dt):
     assert (few[:10] == 0).all() and few[10:].isnan().all()
 
 
+@gpu
+@pytest.mark.parametrize("hd", [64, 128])
+def test_prompt_attention_over_the_range_of_bf16(hd):
+    """Values up to bf16's largest and down to 2^-90, for flat weights and for
+    scores that rise along the keys."""
+    P = _api()
+    g = _gen(hd)
+    lens = [1400, 3, 130]
+    cu, T = _cu(lens), sum(lens)
+    q, k, v = (torch.randn(T, h, hd, generator=g, device="cuda").bfloat16() for h in (2, 1, 1))
+    q = q.abs()
+    rise = (k.abs() * torch.linspace(0.1, 3, T, device="cuda")[:, None, None]).bfloat16()
+    v = v.clamp(-3, 3) / 3
+    for keys in (k, rise):
+        for size in (0.9 * torch.finfo(torch.bfloat16).max, 2.0 ** 115, 2.0 ** -90):
+            vv = (v.double() * size).bfloat16()
+            got = P.prompt_attention(q, keys, vv, cu)
+            want, mag = _prompt64(q, keys, vv, cu.tolist(), cu.tolist(), hd ** -0.5)
+            assert ((got.double() - want).abs() <= (2.5 * HALF_STEP[torch.bfloat16] + 1.6e-5) * mag).all(), size
+
+
 # ---- the draw ---------------------------------------------------------------------
 def _draw64(logits, u, t, k, p, m):
     """One row, in Python's and torch's fp64, entry by entry."""

@@ -53,7 +53,6 @@ constexpr int kCtasPerSm = 2;
 // steps that starting a row is worth (2, 4, 8: 64 sequences of 300 to 4096 in bf16 72.7, 67.2, 69.5 us;
 // 8 of 9001 to 32768 in 2bit_asym 72.6, 70.4, 72.3)
 constexpr int kSetup = 4;
-constexpr float kLift = 14.f;   // log2 of the largest weight p; p s_v stays below 2^15
 constexpr int kRing = 25600;     // bytes of a warp's ring, at most
 
 struct AttnArgs {
@@ -72,6 +71,9 @@ struct Mode {
   static constexpr bool kBf16 = MODE == PF_KV_BF16, k16 = kBf16 || MODE == PF_KV_F16;
   static constexpr bool k2 = MODE == PF_KV_2BIT || MODE == PF_KV_2BIT_ASYM, kAsym = MODE == PF_KV_2BIT_ASYM;
   static constexpr int kTerms = kBf16 ? 3 : 2;
+  // log2 of the largest weight p.  Two fp16 terms want it high: p s_v stays below 2^15.  bf16 terms reach as far as
+  // fp32, and so do bf16 values: sums over a million of the largest stay finite.
+  static constexpr float kLift = kBf16 ? -20.f : 14.f;
 };
 
 template <int HD, int MODE, int PK>
@@ -572,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_kernel(const 
         float w[J][2][2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float top = (m[e] == -INFINITY ? 0.f : m[e]) - kLift;
+          const float top = (m[e] == -INFINITY ? 0.f : m[e]) - M::kLift;
 #pragma unroll
           for (int j = 0; j < J; ++j)
 #pragma unroll

@@ -487,6 +487,26 @@ def test_paged_attention_long_sums(mode):
     assert float((got.double() - want).norm() / want.norm()) < 1e-5
 
 
+@gpu
+@pytest.mark.parametrize("nh", [4, 8])
+def test_paged_attention_over_the_range_of_bf16(nh):
+    """bf16 pages with values up to bf16's largest and down to 2^-90."""
+    P = _api()
+    g = _gen(nh)
+    lens = [1, 50, 3000, 20000]
+    pages = _filled(P, "bf16", 400, 64, 1, 128, g, spread=0.0)
+    unit = (pages.v.float().clamp(-3, 3) / 3).double()
+    table = _block_table(lens, 64, 400, g)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn(4, nh, 128, generator=g, device="cuda")
+    for size in (0.9 * torch.finfo(torch.bfloat16).max, 2.0 ** 115, 2.0 ** -90):
+        for flat in (False, True):  # flat: one sign, so that the sums grow with the length
+            pages.v.copy_((unit.abs() if flat else unit) * size)
+            for scale in (0.0, 128 ** -0.5):
+                want, mag = _attend64(pages, q, table, lens, scale)
+                _near(P.paged_attention(q, pages, table, lens_t, scale=scale), want, mag, 1.6e-5)
+
+
 # ---- prompts ------------------------------------------------------------------------
 def _prompt64(q, k, v, cq, ck, scale):
     out, mag = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))

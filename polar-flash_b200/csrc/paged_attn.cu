@@ -112,6 +112,9 @@ __device__ __forceinline__ uint32_t b2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// The maximum that a part of a row is joined by: maxima pass NaN scores over, the sum of weights does not.  A part
+// of nothing but NaN would have the maximum -inf, and be left out as one without positions.
+__device__ __forceinline__ float marked(float m, float l) { return l != l ? l : m; }
 // Term `n` of x as a sum of 16-bit values, each the rounded rest of those before.
 template <bool BF16>
 __device__ __forceinline__ float term(float x, int n) {
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_kernel(const 
           if (PK == 1 || t < 2) rec[dim] = y * __uint_as_float((unsigned)(127 - sh) << 23) + zs[e];
         }
       if (g == 0 && (PK == 1 || t < 2)) {
-        rec[HD] = m[e];
+        rec[HD] = marked(m[e], l[e]);
         rec[HD + 1] = l[e];
       }
     }
@@ -729,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_kernel(const 
         }
       }
       if (!whole && lane == 0) {
-        a.records[((size_t)record * kHeads + h) * (HD + 2) + HD] = top;
+        a.records[((size_t)record * kHeads + h) * (HD + 2) + HD] = marked(top, ls);
         a.records[((size_t)record * kHeads + h) * (HD + 2) + HD + 1] = ls;
       }
     }

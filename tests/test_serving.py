@@ -507,6 +507,39 @@ def test_paged_attention_over_the_range_of_bf16(nh):
                 _near(P.paged_attention(q, pages, table, lens_t, scale=scale), want, mag, 1.6e-5)
 
 
+@gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("nh,hd", [(4, 128), (8, 64)])
+def test_paged_attention_hands_nan_on(mode, nh, hd):
+    """A NaN in a query head, or in a key that a sequence sees, makes NaN of the
+    heads that meet it, whichever warp and block has it, and of no others."""
+    P = _api()
+    g = _gen(nh)
+    lens = [1, 17, 130, 9000, 0]
+    pages = _filled(P, mode, 200, 64, 2, hd, g, spread=0.3)
+    table = _block_table(lens, 64, 200, g)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn(5, nh, hd, generator=g, device="cuda")
+    clean = P.paged_attention(q, pages, table, lens_t)
+    bad = q.clone()
+    bad[:, 1, 3] = math.nan
+    got = P.paged_attention(bad, pages, table, lens_t)
+    assert got[:4, 1].isnan().all() and (got[4] == 0).all()
+    keep = [h for h in range(nh) if h != 1]
+    assert torch.equal(got[:, keep], clean[:, keep])
+    for b, pos in ((0, 0), (1, 0), (1, 16), (2, 129), (3, 0), (3, 4444), (3, 8999)):
+        page, slot = int(table[b, pos // 64]), pos % 64
+        rows = pages.k if mode in ("fp16", "bf16") else pages.k_scales
+        was = rows[page, 1, slot].clone()
+        rows[page, 1, slot] = math.nan
+        got = P.paged_attention(q, pages, table, lens_t)
+        rows[page, 1, slot] = was
+        want = clean.clone()
+        want[b, nh // 2:] = math.nan
+        assert torch.equal(got.isnan(), want.isnan()), (b, pos)
+        assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)), (b, pos)
+
+
 # ---- prompts ------------------------------------------------------------------------
 def _prompt64(q, k, v, cq, ck, scale):
     out, mag = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))

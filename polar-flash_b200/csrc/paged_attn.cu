@@ -530,9 +530,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_kernel(const 
                 kz = fmaf(1.5f, ksc, meta[32 + g + 8 * i]);
                 vz[j][i] = fmaf(1.5f, vsc[j][i], meta[48 + g + 8 * i]);
               }
-              // the exponent of a positive scale; the quantizer's smallest is 1e-8, less (a row never
-              // written) only makes the weight small
-              up[j][i] = (float)max((int)(__float_as_uint(vsc[j][i]) >> 23) - 127, -30);
+              // the exponent of a positive scale (of what the codes' middle stands for, where that is larger: p z has
+              // to stay in range too); the quantizer's smallest is 1e-8, less (a row never written) only makes the
+              // weight small
+              const float size = M::kAsym ? fmaxf(vsc[j][i], fabsf(vz[j][i])) : vsc[j][i];
+              up[j][i] = (float)max((int)(__float_as_uint(size) >> 23) - 127, -30);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {

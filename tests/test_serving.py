@@ -540,6 +540,27 @@ def test_paged_attention_hands_nan_on(mode, nh, hd):
         assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)), (b, pos)
 
 
+@gpu
+@pytest.mark.parametrize("nh", [4, 8])
+def test_paged_attention_of_rows_that_hardly_vary(nh):
+    """2bit_asym rows whose zero is up to 2^130 times their scale (a constant row's
+    scale is 1e-8, whatever its value is), beside ordinary ones."""
+    P = _api()
+    g = _gen(nh)
+    lens = [1, 40, 700, 5000]
+    pages = _filled(P, "2bit_asym", 120, 64, 1, 128, g, spread=0.0)
+    table = _block_table(lens, 64, 120, g)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = torch.randn(4, nh, 128, generator=g, device="cuda")
+    zeros, scales = pages.v_zeros.clone(), pages.v_scales.clone()
+    for size in (1.0, 1e10, 1e30, -1e30):
+        for every in (1, 3):
+            pages.v_zeros.copy_(zeros), pages.v_scales.copy_(scales)
+            pages.v_zeros[:, :, ::every], pages.v_scales[:, :, ::every] = size, 1e-8
+            want, mag = _attend64(pages, q, table, lens, 128 ** -0.5)
+            _near(P.paged_attention(q, pages, table, lens_t), want, mag, 1.6e-5)
+
+
 # ---- prompts ------------------------------------------------------------------------
 def _prompt64(q, k, v, cq, ck, scale):
     out, mag = (torch.zeros(q.shape, dtype=torch.float64, device="cuda") for _ in range(2))

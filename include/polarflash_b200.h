@@ -458,11 +458,17 @@ PF_API int pf_paged_attention(const pf_kv_pages* pages, const void* q, int dtype
  * before they meet v; a NaN or infinity reaches the rows that see its key only
  * (rows that share a tile with one in v are computed again, slowly).  scale > 0.
  * status (device int32, may be NULL) receives PF_ERR_TIMEOUT, and rows of out
- * NaN, when a bounded wait of the kernel gave up; it is not written otherwise. */
+ * NaN, when a bounded wait of the kernel gave up; it is not written otherwise.
+ * pf_prompt_status reports the same for all calls on the current device. */
 PF_API int pf_prompt_attention(const void* q, long long q_stride, const void* k, long long k_stride, const void* v,
                                long long v_stride, void* out, long long out_stride, int dtype, const int* cu_q,
                                const int* cu_k, int seqs, int total_q, int total_k, int n_heads, int n_kv_heads,
                                int head_dim, float scale, int* status, void* stream);
+/* *status receives PF_OK, or PF_ERR_TIMEOUT where a wait of a
+ * pf_prompt_attention kernel on the current device has given up since the last
+ * reset (captured calls and other streams' included), after the work queued on
+ * `stream`, which the call synchronises; `reset` non-zero clears it. */
+PF_API int pf_prompt_status(int reset, int* status, void* stream);
 /* pf_prompt_attention with waits that give up after wait_ns (0 to 2e9) instead
  * of two seconds: 0 gives up wherever a warp has to wait at all.  Rows of out
  * are what pf_prompt_attention gives or, where their block gave up, NaN; status

@@ -259,6 +259,10 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What waits that gave up left on a device (pf_prompt_status): in the library's
+// own image, so that every call reports to it, captured ones too.
+static __device__ unsigned g_prompt_status;
+
 // What a CTA works on: sequence rows, and per tile its head, first row and
 // number of key tiles.
 struct Job {
@@ -584,7 +588,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && tiles > 0) ok = __all_sync(0xffffffffu, wait(obar + 8 * t, (tiles - 1) & 1));
       if (!ok) {
         abort_flag = 1;
-        if (lane == 0 && a.status) atomicExch(a.status, (unsigned)PF_ERR_TIMEOUT);
+        if (lane == 0) {
+          atomicExch(&g_prompt_status, (unsigned)PF_ERR_TIMEOUT);
+          if (a.status) atomicExch(a.status, (unsigned)PF_ERR_TIMEOUT);
+        }
       }
       fence_after();
       T* out = static_cast<T*>(a.out) + (long long)(job.q0 + row) * a.os + (long long)head * a.hd;
@@ -753,4 +760,21 @@ int pf_prompt_selftest(const void* q, long long q_stride, const void* k, long lo
   if (wait_ns > kWaitNs) return PF_ERR_INVALID_ARGUMENT;
   return prompt_attention(q, q_stride, k, k_stride, v, v_stride, out, out_stride, dtype, cu_q, cu_k, seqs, total_q,
                           total_k, n_heads, n_kv_heads, head_dim, scale, status, 0, wait_ns, stream);
+}
+
+int pf_prompt_status(int reset, int* status, void* stream) {
+  if (!status) return PF_ERR_INVALID_ARGUMENT;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  unsigned word = 0;
+  cudaError_t e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbolAsync(&word, g_prompt_status, sizeof(word), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess && reset && word) {
+    const unsigned zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_prompt_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  }
+  if (e != cudaSuccess) return report_cuda(e);
+  *status = (int)word;
+  return PF_OK;
 }

@@ -47,7 +47,7 @@ EXPORTS = (
     "pf_decode_attention_compressed", "pf_workspace_status", "pf_qlinear_noalloc_status", "pf_wait_selftest",
     "pf_peer_export", "pf_peer_open", "pf_peer_close", "pf_qlinear_group_gather", "pf_peers_wait",
     "pf_allgather_rows", "pf_kv_pages_check", "pf_paged_rope_kv", "pf_paged_attention_workspace_size",
-    "pf_paged_attention", "pf_prompt_attention", "pf_prompt_selftest", "pf_sample_logits",
+    "pf_paged_attention", "pf_prompt_attention", "pf_prompt_status", "pf_prompt_selftest", "pf_sample_logits",
 )
 
 
@@ -203,6 +203,8 @@ def load():
     L.pf_paged_attention.argtypes = [PAGES, P, I, P, P, I, P, I, I, F, P, SZ, P]
     L.pf_prompt_attention.restype = I
     L.pf_prompt_attention.argtypes = [P, LL, P, LL, P, LL, P, LL, I, P, P, I, I, I, I, I, I, F, P, P]
+    L.pf_prompt_status.restype = I
+    L.pf_prompt_status.argtypes = [I, ctypes.POINTER(I), P]
     L.pf_prompt_selftest.restype = I
     L.pf_prompt_selftest.argtypes = [P, LL, P, LL, P, LL, P, LL, I, P, P, I, I, I, I, I, I, F, P, ctypes.c_uint64, P]
     L.pf_sample_logits.restype = I

@@ -276,30 +276,15 @@ def paged_attention(q: torch.Tensor, pages: KVPages, block_table: torch.Tensor, 
     return out
 
 
-_status_words = {}
-
-
-def _status_word(index: int) -> Optional[torch.Tensor]:
-    """The device's status word; None where the first call is being captured
-    (a tensor made there would belong to the graph)."""
-    t = _status_words.get(index)
-    if t is None and not torch.cuda.is_current_stream_capturing():
-        t = _status_words[index] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{index}")
-        torch.cuda.current_stream(index).synchronize()  # other streams' kernels write it too
-    return t
-
-
 def check_serving_status(device) -> None:
     """Raises RuntimeError when a bounded wait of a prompt_attention kernel on
-    `device` gave up since the last check (its rows are NaN then).  Waits for
-    the device's current stream."""
+    `device` gave up since the last check (its rows are NaN then), in a replayed
+    graph too.  Waits for the device's current stream."""
     device = torch.device(device)
-    t = _status_words.get(torch.cuda.current_device() if device.index is None else device.index)
-    if t is not None:
-        st = int(t.item())
-        if st != _lib.OK:
-            t.zero_()
-            _lib.check(st, "pf_prompt_attention")
+    index = torch.cuda.current_device() if device.index is None else device.index
+    st = ctypes.c_int(_lib.OK)
+    _call(_lib.load().pf_prompt_status, "pf_prompt_status", index, 1, ctypes.byref(st))
+    _lib.check(st.value, "pf_prompt_attention")
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
@@ -349,7 +334,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if T and B:
         _call(_lib.load().pf_prompt_attention, "pf_prompt_attention", dev, q.data_ptr(), qs, k.data_ptr(), ks,
               v.data_ptr(), vs, out.data_ptr(), os, _DTYPES[dtype], cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
-              B, T, TK, nh, nkv, hd, hd ** -0.5 if scale is None else float(scale), _ptr(_status_word(dev)))
+              B, T, TK, nh, nkv, hd, hd ** -0.5 if scale is None else float(scale), None)
     return out
 
 

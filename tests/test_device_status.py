@@ -84,6 +84,7 @@ def test_prompt_attention_that_gives_up_leaves_nothing_behind(hd, wait_ns):
     behind on the same multiprocessors, whose shared memory a copy still in
     flight would have overwritten, and later calls give what they give alone."""
     from polarflash_b200 import _lib, prompt_attention
+    from polarflash_b200.serving import check_serving_status
 
     g = torch.Generator(device="cuda").manual_seed(hd)
     lens = [700, 90, 1, 1500, 300] * 4
@@ -110,6 +111,51 @@ def test_prompt_attention_that_gives_up_leaves_nothing_behind(hd, wait_ns):
         assert int(status) == (_lib.ERR_TIMEOUT if gone.any() else _lib.OK)
         if wait_ns == 0:
             assert gone.any()
+        if gone.any():
+            with pytest.raises(RuntimeError, match="timed out"):
+                check_serving_status("cuda")
+        check_serving_status("cuda")
         status.zero_()
     _lib.check(limited(out, 2_000_000_000), "pf_prompt_selftest")
     assert torch.equal(out, want) and int(status) == _lib.OK
+
+
+def _captured_first_call(out):
+    """In a fresh process: the device's first prompt_attention is captured; each
+    replay that gives up is reported once, by whichever stream asks."""
+    import polarflash_b200 as P
+    from polarflash_b200 import _lib
+    from polarflash_b200.serving import check_serving_status
+
+    q = torch.randn(300, 2, 64, device="cuda").half()
+    cu = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    L = _lib.load()
+    L.pf_prompt_attention = lambda *a: L.pf_prompt_selftest(*a[:-1], 0, a[-1])
+    s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s):
+        P.prompt_attention(q, q, q, cu)
+    said = []
+    for _ in range(2):
+        with torch.cuda.stream(s):
+            g.replay()
+            for _ in range(2):
+                try:
+                    check_serving_status("cuda")
+                    said.append("ok")
+                except RuntimeError as e:
+                    said.append(str(e))
+    out.put(said)
+
+
+def test_captured_first_call_that_gives_up_is_reported():
+    import torch.multiprocessing as mp
+
+    ctx = mp.get_context("spawn")
+    out = ctx.Queue()
+    p = ctx.Process(target=_captured_first_call, args=(out,))
+    p.start()
+    said = out.get(timeout=120)
+    p.join(60)
+    assert p.exitcode == 0
+    assert "timed out" in said[0] and "timed out" in said[2] and said[1] == said[3] == "ok"

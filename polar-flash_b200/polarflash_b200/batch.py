@@ -159,7 +159,8 @@ class BatchDecoder:
     def add(self, prompts: Sequence[torch.Tensor]):
         """Starts a sequence for each prompt (1-D token ids of the vocabulary, not
         empty) in a free slot: (slots, logits [len(prompts), vocab] of the
-        prompts' last tokens).  Refused as a whole where slots or pages lack."""
+        prompts' last tokens).  Refused as a whole where slots or pages lack; taken
+        back, with RuntimeError, where a wait of the prompts' attention gave up."""
         ids = [p.reshape(-1).to(self.device, torch.long) for p in prompts]
         lens = [len(i) for i in ids]
         free = [i for i, n in enumerate(self.lengths) if n == 0]
@@ -178,7 +179,9 @@ class BatchDecoder:
             raise ValueError(f"token ids {lo}..{hi}: 0 to {self.embed.shape[0] - 1}")
         slots = free[:len(ids)]
         try:
-            return self._add(slots, packed, lens)
+            out = self._add(slots, packed, lens)
+            check_serving_status(self.device)
+            return out
         except BaseException:
             for s in slots:
                 self.release(s)

@@ -145,6 +145,28 @@ def test_batch_decoder_slots_and_pages():
         full.step(tok)
 
 
+def _give_up(monkeypatch):
+    """prompt_attention's kernel gives up wherever it has to wait."""
+    from polarflash_b200 import _lib
+
+    L = _lib.load()
+    monkeypatch.setattr(L, "pf_prompt_attention", lambda *a: L.pf_prompt_selftest(*a[:-1], 0, a[-1]))
+
+
+@gpu
+def test_prompts_whose_attention_gave_up_are_taken_back(monkeypatch):
+    _, d = _parts()
+    b = _batch(d)
+    want = b.add([torch.tensor(PROMPTS[0])])[1]
+    with monkeypatch.context() as m:
+        _give_up(m)
+        with pytest.raises(RuntimeError, match="timed out"):
+            b.add([torch.tensor(p) for p in PROMPTS[1:3]])
+    assert b.active() == [0] and len(b.allocator) == 12 - 2 and b._lens.tolist() == [20, 0, 0, 0]
+    slots, got = b.add([torch.tensor(PROMPTS[0])])  # nothing is left to report
+    assert slots == [1] and torch.equal(got, want)
+
+
 @gpu
 def test_generate():
     """Greedy tokens are the argmax of the steps' logits, batch and single

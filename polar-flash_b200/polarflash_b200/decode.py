@@ -33,7 +33,7 @@ import torch.nn.functional as F
 from . import _lib
 from .kv_cache import KV_MODES, kv_row_bytes
 from .qweight import QWeight, group_workspace_bytes, qlinear, qlinear_multi
-from .serving import prompt_attention, sample_logits
+from .serving import check_serving_status, prompt_attention, sample_logits
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -194,7 +194,9 @@ class PFlashDecoder:
     # ---- eager forward (prefill, or any number of new tokens) --------------
     def forward(self, input_ids: torch.Tensor) -> torch.Tensor:
         """Logits [S, vocab] for the S new tokens `input_ids` (1-D, on the
-        device), appended after the tokens already in the cache."""
+        device), appended after the tokens already in the cache.  Under
+        prompt_dtype several tokens are waited for: RuntimeError where a wait of
+        their attention gave up, and the tokens are not appended."""
         ids = input_ids.reshape(-1).to(self.device)
         S, start = ids.shape[0], self.length
         if start + S > self.max_seq:
@@ -228,6 +230,8 @@ class PFlashDecoder:
         cs = self._rope_cs(pos)
         for li in range(len(self.layers)):
             h = self._layer(li, h, cs, attend, ws)
+        if fused:
+            check_serving_status(self.device)
         self.length = T
         return self._head(self._rmsnorm(h, self.final_norm))
 

@@ -231,3 +231,23 @@ def test_prompt_dtype_of_the_single_decoder(dt, tol, kv):
 
     with pytest.raises(ValueError):
         PFlashDecoder(CFG, a.layers, a.embed, a.final_norm, a.lm_head, 8, prompt_dtype=torch.float32)
+
+
+@gpu
+def test_prompt_dtype_that_gave_up_raises(monkeypatch):
+    from test_decode_step import _decoder
+
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    d = _decoder(dm.build())
+    d.prompt_dtype = torch.bfloat16
+    ids = torch.tensor(dm.PROMPT, device="cuda")
+    want = d.forward(ids[:9]).clone()
+    with monkeypatch.context() as m:
+        _give_up(m)
+        for call in (lambda: d.forward(ids[9:]), lambda: d.generate(ids[9:], 3)):
+            with pytest.raises(RuntimeError, match="timed out"):
+                call()
+            assert d.length == 9
+    d.length = 0
+    assert torch.equal(d.forward(ids[:9]), want)

@@ -240,7 +240,8 @@ class PFlashDecoder:
         """The tokens drawn after the prompt `input_ids` (appended to what the
         cache holds): max_new_tokens, or up to and with `eos`; sample_logits'
         parameters, uniform numbers from `generator` (on the device).  Steps
-        replay the captured graph where there is one."""
+        replay the captured graph where there is one.  Under `tp` every rank calls
+        it, and all take the tokens that the first rank draws."""
         out: List[torch.Tensor] = []
         if max_new_tokens < 1:
             return []
@@ -248,6 +249,8 @@ class PFlashDecoder:
         while True:
             u = torch.rand(1, generator=generator, device=self.device)
             tok = sample_logits(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            if self.tp is not None:  # the ranks' generators need not agree
+                tok = self.tp.gather([tok.view(1, 1)])[0][0, :1].contiguous()
             out.append(tok)
             if len(out) == max_new_tokens or (eos is not None and int(tok) == eos):
                 return torch.cat(out).tolist()

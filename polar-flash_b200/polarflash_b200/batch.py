@@ -267,11 +267,20 @@ class BatchDecoder:
         """The tokens drawn after each prompt (sample_logits' parameters, numbers
         for all sequences): max_new_tokens each, or up to and with `eos`.  The
         uniform numbers come from `generator` (on the device).  No other sequence
-        may be active; these are released at the end."""
+        may be active; these are released at the end.  Without `eos` a call that
+        max_seq or the pages cannot hold is refused before it starts; with it a
+        sequence that finds no room for its next token ends there, shorter."""
         if self.active():
             raise RuntimeError("BatchDecoder.generate: other sequences are active")
         if max_new_tokens < 1:
             return [[] for _ in prompts]
+        if eos is None:
+            held = [p.numel() + max_new_tokens - 1 for p in prompts]  # the last token drawn is not cached
+            if held and max(held) > self.max_seq:
+                raise ValueError(f"a sequence of {max(held)} tokens: at most {self.max_seq}")
+            need = sum(-(-n // self.page_size) for n in held)
+            if need > len(self.allocator):
+                raise RuntimeError(f"{need} cache pages needed, {len(self.allocator)} free")
         slots, logits = self.add(prompts)
         kw = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         rand = lambda n: torch.rand(n, generator=generator, device=self.device)  # noqa: E731
@@ -279,6 +288,13 @@ class BatchDecoder:
         tokens = torch.zeros(self.max_seqs, dtype=torch.long, device=self.device)
         drawn = []
         live = set(slots)
+        ends = {}  # tokens of the sequences that found no room
+
+        def full(s):
+            ends[s] = len(drawn)
+            live.discard(s)
+            self.release(s)
+
         try:
             tokens[at] = sample_logits(logits, rand(len(slots)), **kw)
             drawn.append(tokens[at].clone())
@@ -288,6 +304,11 @@ class BatchDecoder:
                         if t == eos and s in live:
                             live.discard(s)
                             self.release(s)
+                    for s in [s for s in slots if s in live and self.lengths[s] >= self.max_seq]:
+                        full(s)
+                    turn = [s for s in slots if s in live and self.lengths[s] % self.page_size == 0]
+                    while len(turn) > len(self.allocator):  # the last one's pages go to the others
+                        full(turn.pop())
                     if not live:
                         break
                 tokens.copy_(sample_logits(self.step(tokens), rand(self.max_seqs), **kw))
@@ -299,4 +320,5 @@ class BatchDecoder:
                 self.release(s)
         if eos is None:
             return rows
+        rows = [r[:ends.get(s)] for s, r in zip(slots, rows)]
         return [r[:r.index(eos) + 1] if eos in r else r for r in rows]

@@ -145,6 +145,41 @@ def test_batch_decoder_slots_and_pages():
         full.step(tok)
 
 
+@gpu
+def test_generate_where_the_room_ends():
+    """max_seq and the pages: refused as a whole beforehand without eos; with one
+    that is not drawn each sequence ends where it finds no room, and the others
+    go on with its pages; what was drawn is what a larger cache gives."""
+    _, d = _parts()
+    prompts = [torch.tensor(p) for p in PROMPTS]  # of 20, 7, 1 and 16 tokens
+    kw = dict(temperature=0.0)
+    big = _batch(d, num_pages=16)
+    want = big.generate(prompts, 30, **kw)
+    never = next(t for t in range(CFG["vocab_size"]) if all(t not in r for r in want))
+    calls = []
+    short = _batch(d, max_seq=24)
+    short.add = lambda p, add=short.add: calls.append(len(p)) or add(p)
+    with pytest.raises(ValueError):
+        short.generate(prompts, 6, **kw)
+    assert not calls and short.generate(prompts, 5, **kw) == [r[:5] for r in want]
+    # 24 positions hold a prompt of n and 24 - n tokens, and one more is drawn
+    assert short.generate(prompts, 30, eos=never, **kw) == [r[: min(30, 25 - len(p))] for r, p in zip(want, PROMPTS)]
+    assert len(short.allocator) == 12 and not short.active()
+    few = _batch(d, num_pages=6)
+    with pytest.raises(RuntimeError):
+        few.generate(prompts, 30, **kw)
+    assert not few.active() and len(few.allocator) == 6
+    # five pages hold the prompts; the fourth needs a second page at once and takes the last; the second, at 16, finds
+    # none and ends with 16 - 7 + 1 tokens, and its page serves the first, at 32
+    got = few.generate(prompts, 30, eos=never, **kw)
+    lens = [len(r) for r in got]
+    assert lens[1] == 10 and max(lens) == 30 and all(r == w[: len(r)] for r, w in zip(got, want))
+    assert len(few.allocator) == 6 and not few.active()
+    stop = want[1][3]
+    cut = few.generate(prompts[1:2], 30, eos=stop, **kw)
+    assert cut == [want[1][: want[1].index(stop) + 1]]
+
+
 def _give_up(monkeypatch):
     """prompt_attention's kernel gives up wherever it has to wait."""
     from polarflash_b200 import _lib

@@ -240,11 +240,16 @@ class PFlashDecoder:
         """The tokens drawn after the prompt `input_ids` (appended to what the
         cache holds): max_new_tokens, or up to and with `eos`; sample_logits'
         parameters, uniform numbers from `generator` (on the device).  Steps
-        replay the captured graph where there is one.  Under `tp` every rank calls
+        replay the captured graph where there is one.  Without `eos` a call that
+        the cache cannot hold is refused before it starts; with it the tokens end
+        where the cache is full.  Under `tp` every rank calls
         it, and all take the tokens that the first rank draws."""
         out: List[torch.Tensor] = []
         if max_new_tokens < 1:
             return []
+        held = self.length + input_ids.numel() + max_new_tokens - 1  # the last token drawn is not cached
+        if eos is None and held > self.max_seq:
+            raise ValueError(f"cache holds {self.max_seq} tokens; {held} requested")
         logits = self.forward(input_ids)[-1:]
         while True:
             u = torch.rand(1, generator=generator, device=self.device)
@@ -252,7 +257,7 @@ class PFlashDecoder:
             if self.tp is not None:  # the ranks' generators need not agree
                 tok = self.tp.gather([tok.view(1, 1)])[0][0, :1].contiguous()
             out.append(tok)
-            if len(out) == max_new_tokens or (eos is not None and int(tok) == eos):
+            if len(out) == max_new_tokens or (eos is not None and (int(tok) == eos or self.length >= self.max_seq)):
                 return torch.cat(out).tolist()
             tok = tok.clamp_min(0)  # -1 is drawn where no logit is above -inf
             logits = self.step(tok) if self._graph is not None else self.forward(tok)

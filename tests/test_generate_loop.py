@@ -1,10 +1,11 @@
-"""PFlashDecoder.generate over column-parallel ranks: every rank takes the first
-rank's tokens, whatever its own generator's state is.  Two gloo ranks on the
-CPU; the model and the draw are stand-ins, the loop and the gather are the
-decoder's own."""
+"""PFlashDecoder.generate's loop on the CPU; the model and the draw are stand-ins.
+Over column-parallel ranks (two gloo ones) every rank takes the first rank's
+tokens, whatever its own generator's state is; a cache that is too small loses
+nothing that was drawn."""
 import os
 import socket
 
+import pytest
 import torch
 import torch.distributed as dist
 import torch.multiprocessing as mp
@@ -29,6 +30,23 @@ def _draw(logits, u, temperature, top_k, top_p, min_p):
     return (u * V).long()
 
 
+def _decoder(decode, tp, fed):
+    d = object.__new__(decode.PFlashDecoder)
+    d.tp, d._graph, d.device, d.max_seq, d.length = tp, None, torch.device("cpu"), 64, 0
+
+    def forward(ids):
+        fed.append(ids.tolist())
+        if tp is not None:
+            tp.gather([torch.zeros(1, 3)])  # a projection's: a rank that left the loop would be missed here
+        if d.length + len(ids) > d.max_seq:
+            raise ValueError("cache")
+        d.length += len(ids)
+        return _logits(ids)
+
+    d.forward = forward
+    return d
+
+
 def _worker(rank, world, port, eos, out_q):
     import sys
     from datetime import timedelta
@@ -42,17 +60,8 @@ def _worker(rank, world, port, eos, out_q):
         from polarflash_b200.parallel import GroupGather
 
         decode.sample_logits = _draw
-        d = object.__new__(decode.PFlashDecoder)
-        d.tp, d._graph, d.device, d.max_seq, d.length = GroupGather(), None, torch.device("cpu"), 64, 0
         fed = []
-
-        def forward(ids):
-            fed.append(ids.tolist())
-            d.tp.gather([torch.zeros(1, 3)])  # a projection's: a rank that left the loop would be missed here
-            d.length += len(ids)
-            return _logits(ids)
-
-        d.forward = forward
+        d = _decoder(decode, GroupGather(), fed)
         gen = torch.Generator().manual_seed(7 + rank)  # a seed per rank
         alone = (torch.rand(12, generator=torch.Generator().manual_seed(7 + rank)) * V).long().tolist()
         out_q.put((rank, d.generate(torch.tensor([3, 1, 4]), 12, eos=eos, generator=gen), fed, alone))
@@ -82,3 +91,19 @@ def test_ranks_with_different_generators_draw_the_same_tokens():
     eos = a[4]
     (_, a2, fed_a, _), (_, b2, fed_b, _) = _run(eos)  # both leave the loop at once
     assert a2 == b2 == a[: a.index(eos) + 1] and fed_a == fed_b
+
+
+def test_where_the_cache_ends(monkeypatch):
+    from polarflash_b200 import decode
+
+    monkeypatch.setattr(decode, "sample_logits", _draw)
+    gen = lambda: torch.Generator().manual_seed(3)  # noqa: E731
+    fed = []
+    want = _decoder(decode, None, []).generate(torch.arange(10), 55, generator=gen())
+    assert len(want) == 55  # 10 + 54 cached
+    d = _decoder(decode, None, fed)
+    with pytest.raises(ValueError):
+        d.generate(torch.arange(10), 56, generator=gen())
+    assert fed == [] and d.length == 0
+    never = next(t for t in range(V + 1) if t not in want)
+    assert d.generate(torch.arange(10), 100, eos=never, generator=gen()) == want and d.length == 64

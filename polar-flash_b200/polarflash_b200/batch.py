@@ -243,6 +243,8 @@ class BatchDecoder:
         act = self.active()
         if tokens.shape != (self.max_seqs,):
             raise ValueError(f"tokens {tuple(tokens.shape)}: [{self.max_seqs}] is needed")
+        if tokens.device != self.device or tokens.is_floating_point() or tokens.is_complex():
+            raise ValueError(f"tokens: token ids on {self.device} are needed, not {tokens.dtype} on {tokens.device}")
         if any(self.lengths[s] >= self.max_seq for s in act):
             raise ValueError(f"a sequence holds {self.max_seq} tokens")
         need = sum(self.lengths[s] % self.page_size == 0 for s in act)

@@ -180,6 +180,24 @@ def test_generate_where_the_room_ends():
     assert cut == [want[1][: want[1].index(stop) + 1]]
 
 
+@gpu
+def test_refused_steps_change_nothing():
+    """Ids on the host, of no integer type or no ids at all: lengths, pages and
+    the device's lengths stay; the next step gives what it gives without them."""
+    _, d = _parts()
+    tok = torch.tensor([11, 12, 13, 14], device="cuda")
+    out = []
+    for bad in ([], [tok.cpu(), tok.float(), tok.half(), tok[:2], tok[None], tok.cpu().int()]):
+        b = _batch(d)
+        b.add([torch.tensor(PROMPTS[3]), torch.tensor(PROMPTS[1])])  # 16 tokens: the next one needs a page
+        for t in bad:
+            with pytest.raises(ValueError):
+                b.step(t)
+            assert b.lengths == [16, 7, 0, 0] and len(b.allocator) == 12 - 2 and b._lens.tolist() == [16, 7, 0, 0]
+        out.append(b.step(tok.int() if bad else tok)[:2].clone())
+    assert torch.equal(*out)
+
+
 def _give_up(monkeypatch):
     """prompt_attention's kernel gives up wherever it has to wait."""
     from polarflash_b200 import _lib

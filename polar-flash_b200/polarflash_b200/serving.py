@@ -84,8 +84,12 @@ class KVPages:
     """One layer's pages: rows k, v [num_pages, kv_heads, page_size, row] (fp16
     / bf16 values, int8 codes, or uint8 bytes of four 2-bit codes) and, for the
     quantized modes, fp32 scales (and zeros, "2bit_asym") [num_pages, kv_heads,
-    page_size], as CompressedKVCache quantizes rows
-    (polarflash_rt/kv_cache/compressed_kv.py:68-150)."""
+    page_size]: the formulas of CompressedKVCache
+    (polarflash_rt/kv_cache/compressed_kv.py:68-150) as torch evaluates them on
+    a CUDA device, where dividing by a number is multiplying by its reciprocal.
+    kv_cache.kv_quantize divides, as on a CPU: its scales differ by at most
+    3 * 2^-24 of themselves, its codes by one where a value lies on the border
+    of two."""
 
     __slots__ = ("mode", "k", "v", "k_scales", "v_scales", "k_zeros", "v_zeros", "num_pages", "kv_heads", "page_size",
                  "head_dim", "index", "desc")

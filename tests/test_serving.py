@@ -305,6 +305,44 @@ def test_cache_write_at_borders(mode):
 
 
 @gpu
+@pytest.mark.parametrize("mode", ["int8", "2bit", "2bit_asym"])
+def test_cache_write_beside_kv_quantize(mode):
+    """How far a paged row is from the contiguous cache's.  The scale is a product
+    with a rounded reciprocal for a quotient: three roundings, 3 * 2^-24 of itself.
+    A code is off by at most one, and only where the value's place, of at most
+    128 steps, is within 128 * 8 * 2^-24 of a border between two (the scales' 3,
+    the quotients' 2, the sum's and the span's)."""
+    P = _api()
+    from polarflash_b200.kv_cache import kv_quantize
+
+    T, nkv, hd = 4096, 2, 128
+    k = torch.randn(T, nkv, hd, generator=_gen(3), device="cuda")
+    k *= torch.exp2(torch.randint(-20, 20, (T, nkv, 1), generator=_gen(4), device="cuda").float())
+    k[:512] = (k[:512] * 64).round() / 64  # many values that are equal parts of the largest
+    pages = P.KVPages.empty(mode, T // 64, 64, nkv, hd, "cuda")
+    table = torch.arange(T // 64, dtype=torch.int32, device="cuda")[None]
+    P.paged_rope_kv(None, k, k, None, None, pages, table, torch.tensor([T], dtype=torch.int32, device="cuda"), _cu([T]))
+    c, s, z = kv_quantize(k, mode)
+    row = lambda t: t.transpose(1, 2).reshape(T, nkv, -1)  # noqa: E731
+    mine, scale = row(pages.k), row(pages.k_scales[..., None])
+    assert ((scale.double() / s.double() - 1).abs() <= 3.01 * 2.0 ** -24).all()
+    x = k.double()
+    if mode == "int8":
+        place, border = x / s.double(), 0.5
+    else:
+        codes = lambda t: torch.stack([(t >> sh & 3) for sh in (6, 4, 2, 0)], -1).flatten(-2)  # noqa: E731
+        c, mine = codes(c), codes(mine)
+        place, border = (x / s.double() + 2, 0.0) if mode == "2bit" else ((x - z.double()) / s.double(), 0.5)
+        if z is not None:
+            assert torch.equal(row(pages.k_zeros[..., None]), z)
+    off = (c.int() - mine.int()).abs()
+    assert int(off.max()) <= 1
+    near = ((place - border) - (place - border).round()).abs() <= 128 * 8 * 2.0 ** -24
+    assert (near | (off == 0)).all()
+    assert int((off > 0).sum()) < 0.001 * off.numel()
+
+
+@gpu
 def test_cache_write_forms():
     """One token per sequence without cu_seqlens; no rotation; no queries; q
     rotated in place; nothing to do; many sequences (the search for a row's

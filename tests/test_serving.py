@@ -652,6 +652,29 @@ def test_prompt_attention(dt, nh, nkv, hd, lens, past):
 
 
 @gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hd", [64, 128, 96])
+def test_prompt_attention_row_norms(dt, hd):
+    """Row by row, normwise: a rounding by half a step e is e / sqrt(6) of its value
+    in the root of the mean square (an error even in -e..e, over values even in a
+    binade).  The weights and the output are rounded once each, and with values of
+    random sign both count alike: 0.58 e, over 4 heads of as many dimensions and at
+    least 64 keys of like weight; below e.  A key too many or too few among n is
+    1 / sqrt(n) of a row's norm: six times the bound for bf16 at 2000 keys."""
+    P = _api()
+    g = _gen(hd)
+    lens, past = [2000, 700, 128], [0, 300, 129]
+    cq, ck = _cu(lens), _cu([a + b for a, b in zip(lens, past)])
+    q = (0.3 * torch.randn(sum(lens), 4, hd, generator=g, device="cuda")).to(dt)
+    k, v = (torch.randn(int(ck[-1]), 2, hd, generator=g, device="cuda").to(dt) for _ in range(2))
+    got = P.prompt_attention(q, k, v, cq, ck)
+    want, _ = _prompt64(q, k, v, cq.tolist(), ck.tolist(), hd ** -0.5)
+    off = (got.double() - want).flatten(1).norm(dim=1) / want.flatten(1).norm(dim=1)
+    keys = torch.cat([torch.arange(p + 1, p + n + 1, device="cuda") for n, p in zip(lens, past)])
+    assert float(off[keys >= 64].max()) < HALF_STEP[dt]
+
+
+@gpu
 def test_prompt_attention_of_many_sequences():
     """100 sequences, some of them empty, of up to 150 queries; keys for some
     only; and no key at all."""

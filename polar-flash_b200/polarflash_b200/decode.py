@@ -99,6 +99,8 @@ class PFlashDecoder:
         self.nh = int(config["num_attention_heads"])
         self.nkv = int(config["num_key_value_heads"])
         self.hd = self.hidden // self.nh
+        if prompt_dtype is not None and (self.hd % 8 or self.hd > 128):
+            raise ValueError(f"prompt_dtype with head_dim {self.hd}: prompt_attention takes multiples of 8 up to 128")
         self.theta = float(config.get("rope_theta", 1000000.0))
         self.eps = float(config.get("rms_norm_eps", 1e-6))
         self.layers = layers

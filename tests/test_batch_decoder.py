@@ -29,6 +29,18 @@ def test_page_allocator():
     assert a.take(0) == []
 
 
+def test_prompt_dtype_is_refused_for_heads_it_does_not_take():
+    from polarflash_b200.decode import PFlashDecoder
+
+    for hd in (136, 20):
+        cfg = dict(CFG, hidden_size=4 * hd)
+        x = torch.zeros(CFG["vocab_size"], 4 * hd)
+        args = (cfg, [], x, x[0], x, 8)
+        PFlashDecoder(*args)
+        with pytest.raises(ValueError):
+            PFlashDecoder(*args, prompt_dtype=torch.bfloat16)
+
+
 def _parts():
     from test_decode_step import _decoder
 

@@ -414,7 +414,7 @@ PF_API int pf_kv_pages_check(const pf_kv_pages* pages);
  * by pf_kv_quantize's formulas, the scale being max|x| (or the span) times the
  * fp32 reciprocal of 127, 1.75 or 3, as the reference's tensor expression is
  * evaluated on a CUDA device (pf_kv_quantize takes the quotient, as on a CPU;
- * 16-bit rows: rounded once).  q_out [tokens][n_heads]
+ * 16-bit rows: rounded once; a row with a NaN has a NaN scale).  q_out [tokens][n_heads]
  * [head_dim] (NULL with q NULL, n_heads 0: only the cache is written; it may be
  * q itself when the types agree and q is contiguous) and, unless NULL, k_out
  * and v_out [tokens][n_kv_heads][head_dim] receive the rotated q, k and the v

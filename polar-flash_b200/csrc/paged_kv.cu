@@ -89,6 +89,19 @@ __device__ __forceinline__ int seq_of(const int* __restrict__ cu, int seqs, int 
   return min(lo, seqs);
 }
 
+// Maxima and minima that hand NaN on, as the tensor expression's do: a row with a
+// NaN has a NaN scale, and reads back as NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 template <int HD, int MODE>
 __device__ __forceinline__ void write_row(const KvPages& pg, bool key, size_t row, const float (&x)[HD / 32]) {
   constexpr int V = HD / 32;
@@ -102,19 +115,19 @@ __device__ __forceinline__ void write_row(const KvPages& pg, bool key, size_t ro
     float lo = INFINITY, hi = MODE == PF_KV_2BIT_ASYM ? -INFINITY : 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      hi = fmaxf(hi, MODE == PF_KV_2BIT_ASYM ? x[i] : fabsf(x[i]));
-      lo = fminf(lo, x[i]);
+      hi = max_nan(hi, MODE == PF_KV_2BIT_ASYM ? x[i] : fabsf(x[i]));
+      lo = min_nan(lo, x[i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-      hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-      if (MODE == PF_KV_2BIT_ASYM) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      if (MODE == PF_KV_2BIT_ASYM) lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     }
     // times the fp32 reciprocal, as torch divides by a number on a CUDA device (pf_kv_quantize
     // takes the quotient: its scale may be one rounding away)
-    const float s = MODE == PF_KV_INT8   ? fmaxf(__fmul_rn(hi, 1.f / 127.f), 1e-8f)
-                    : MODE == PF_KV_2BIT ? fmaxf(__fmul_rn(hi, 1.f / 1.75f), 1e-8f)
-                                         : fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.f / 3.f), 1e-8f);
+    const float s = MODE == PF_KV_INT8   ? max_nan(__fmul_rn(hi, 1.f / 127.f), 1e-8f)
+                    : MODE == PF_KV_2BIT ? max_nan(__fmul_rn(hi, 1.f / 1.75f), 1e-8f)
+                                         : max_nan(__fmul_rn(__fsub_rn(hi, lo), 1.f / 3.f), 1e-8f);
     unsigned code = 0;  // the lane's V codes, packed as the row stores them
 #pragma unroll
     for (int i = 0; i < V; ++i) {

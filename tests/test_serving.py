@@ -305,6 +305,33 @@ def test_cache_write_at_borders(mode):
 
 
 @gpu
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_cache_write_hands_nan_on(mode, hd):
+    """A row with a NaN in any place reads back as NaN (16-bit rows: in that place),
+    and so does what attends to it; the rows beside it are what they are without."""
+    P = _api()
+    g = _gen(hd)
+    T, nkv = 200, 2
+    k, v = (torch.randn(T, nkv, hd, generator=g, device="cuda") for _ in range(2))
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    lens = torch.tensor([T], dtype=torch.int32, device="cuda")
+    clean, pages = (P.KVPages.empty(mode, 4, 64, nkv, hd, "cuda") for _ in range(2))
+    P.paged_rope_kv(None, k, v, None, None, clean, table, lens, _cu([T]))
+    at = (torch.arange(0, T, 3, device="cuda"), torch.arange(0, T, 3, device="cuda") % nkv)
+    place = torch.arange(len(at[0]), device="cuda") % hd
+    k[(*at, place)], v[(*at, hd - 1 - place)] = math.nan, math.nan
+    P.paged_rope_kv(None, k, v, None, None, pages, table, lens, _cu([T]))
+    for which, x in (("k", k), ("v", v)):
+        got, was = (_values(t, which).transpose(1, 2).reshape(256, nkv, hd)[:T] for t in (pages, clean))
+        want = x.isnan() if mode in ("fp16", "bf16") else x.isnan().any(-1, keepdim=True).expand_as(x)
+        assert torch.equal(got.isnan(), want), which
+        assert torch.equal(got[~want], was[~want]), which
+    q = torch.randn(1, 2, hd, generator=g, device="cuda")
+    assert P.paged_attention(q, pages, table, lens).isnan().all()
+
+
+@gpu
 @pytest.mark.parametrize("mode", ["int8", "2bit", "2bit_asym"])
 def test_cache_write_beside_kv_quantize(mode):
     """How far a paged row is from the contiguous cache's.  The scale is a product

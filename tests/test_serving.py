@@ -1101,3 +1101,49 @@ def test_serving_ops_on_streams_and_in_graphs():
         for a, b in zip(outs[i % 2], want[i]):
             assert torch.equal(a, b), i
     torch.cuda.synchronize()
+
+
+@gpu
+def test_serving_ops_beyond_32_bits():
+    """Rows whose offsets pass 2^31 elements and 2^32 bytes: pages at the end of a
+    large cache, strided prompts and logits; each as over compact copies."""
+    P = _api()
+    g = _gen(12)
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB of free device memory")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    # pages: 256 slots of 8 heads of 128, 2^18 elements each; 8300 of them pass 2^31
+    nh, nkv, hd, N = 16, 8, 128, 8300
+    lens = [300, 5, 256]
+    table, near = i32([[N - 1, 0], [N - 3, -1], [8192, -1]]), i32([[0, 1], [2, -1], [3, -1]])
+    T = sum(lens)
+    x = [torch.randn(T, h, hd, generator=g, device="cuda") for h in (nh, nkv, nkv)]
+    q = torch.randn(3, nh, hd, generator=g, device="cuda")
+    for mode in ("bf16", "int8"):
+        far, small = (P.KVPages.empty(mode, n, 256, nkv, hd, "cuda") for n in (N, 4))
+        for pages, t in ((far, table), (small, near)):
+            P.paged_rope_kv(*x, None, None, pages, t, i32(lens), _cu(lens))
+        for which in ("k", "v"):
+            assert torch.equal(getattr(far, which)[table[:, 0].long()], getattr(small, which)[near[:, 0].long()])
+        assert torch.equal(P.paged_attention(q, far, table, i32(lens)), P.paged_attention(q, small, near, i32(lens)))
+        del far
+    # rows 2^23 elements apart
+    wide = torch.empty(300, 1 << 23, dtype=torch.bfloat16, device="cuda")
+    parts = [torch.randn(300, h, hd, generator=g, device="cuda").bfloat16() for h in (nh, nkv, nkv, nh)]
+    at, views = 0, []
+    for p in parts:
+        views.append(wide[:, at:at + p.shape[1] * hd].unflatten(1, (-1, hd)))
+        views[-1].copy_(p)
+        at += p.shape[1] * hd
+    cu = _cu([130, 170])
+    P.prompt_attention(*views[:3], cu, out=views[3])
+    assert torch.equal(views[3], P.prompt_attention(*parts[:3], cu))
+    small, other = (P.KVPages.empty("int8", 4, 256, nkv, hd, "cuda") for _ in range(2))
+    a = P.paged_rope_kv(*views[:3], None, None, small, near, i32([130, 170, 0]), _cu([130, 170, 0]))[0]
+    b = P.paged_rope_kv(*parts[:3], None, None, other, near, i32([130, 170, 0]), _cu([130, 170, 0]))[0]
+    assert torch.equal(a, b) and torch.equal(small.k, other.k) and torch.equal(small.v, other.v)
+    logits = wide[:, :5000].copy_(3 * torch.randn(300, 5000, generator=g, device="cuda"))
+    u = torch.rand(300, generator=g, device="cuda")
+    kw = dict(temperature=0.8, top_k=50, top_p=0.9)
+    assert torch.equal(P.sample_logits(logits, u, **kw), P.sample_logits(logits.contiguous(), u, **kw))

@@ -435,7 +435,9 @@ PF_API int pf_paged_rope_kv(const pf_kv_pages* pages, const void* q, long long q
  * h / (n_heads / n_kv_heads).  q and out [seqs][n_heads][head_dim] contiguous,
  * both of `dtype`, 16-byte aligned; block_table device int32
  * [seqs][table_width].  A sequence of length 0 (or below) gives zeros;
- * positions in a page outside 0..num_pages - 1 are left out, as if masked.
+ * positions in a page outside 0..num_pages - 1 are left out, as if masked.  A
+ * NaN or infinity in q, or in a row that the sequence sees, makes NaN or
+ * infinity of the values that it reaches, and of no others.
  * Sums and softmax statistics are held in fp32.  The workspace (device,
  * 16-byte aligned, contents ignored and overwritten) has at least
  * pf_paged_attention_workspace_size bytes, queried with the target device

@@ -22,8 +22,11 @@
 // they are.  The fp32 operands on the other side keep their
 // precision as sums of 16-bit terms: two fp16 ones, scaled by powers of two to
 // just below fp16's largest value, so that what is a 2^-17th of the largest
-// still has 22 bits, or three bf16 ones.  Up to four query heads per KV head share the eight columns
-// between two terms, more take a product per term.
+// still has 22 bits, or three bf16 ones.  (q beside 2-bit codes stays below
+// 2^13, and a 2^-8th of the largest has 22 bits wherever its code stands.)  Up to
+// four query heads per KV head share the eight columns between two terms, more
+// take a product per term; more than eight are units of their own, which read
+// the row's cache again.
 // A quantized row's value is s c + z (c a centred code), so  q . k = s_k (q . c) +
 // z_k sum q  and  sum p v = sum (p s_v) c + sum p z_v: scales and zeros never
 // touch the tiles.
@@ -31,12 +34,13 @@
 // range while rows differ in scale.
 //
 // Device time: 64 sequences of 300 to 4096 positions in bf16 pages, 32 heads
-// over 8, 67 us (5.7 TB/s, 0.88 of the copy rate: bound by memory); 8 of 9001
-// to 32768 in 2bit_asym, 64 heads over 8, 70 us (1.5 TB/s: bound by the
-// instructions that turn codes into operands, about 500 a tile in all, 0.55
-// issued a cycle and scheduler); one
-// of 2048 in int8 10.6 us (latency).  16-bit stages hold one tile of heads of
-// 128 (8 KB), all others two.
+// over 8, 67 us (5.7 TB/s, 0.88 of the copy rate: bound by memory); the same in
+// int8 58 us (3.5 TB/s); 8 of 9001 to 32768 in 2bit_asym, 64 heads over 8, 70 us
+// (1.5 TB/s).  Quantized rows are bound by the instructions that turn codes into
+// operands, 2 bits about 500 a tile in all, with two warps a scheduler that
+// each issue one in 3.5 (2 bits) or 4.2 (int8) cycles.  One of 2048 in int8 takes
+// 10.6 us (latency).  16-bit stages hold one tile of heads of 128 (8 KB), all
+// others two.
 #include <math.h>
 
 #include "common.cuh"
@@ -403,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) paged_attn_kernel(const 
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
           sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        // 2^e with top 2^-e in [2^14, 2^15) (2-bit codes: [2^6, 2^7), q is multiplied by up to 2^8
+        // 2^e with top 2^-e in [2^14, 2^15) (2-bit codes: [2^6, 2^7), q is multiplied by up to 2^6
         // there); 1 for bf16, whose terms reach as far as fp32
         int e = 0;
         if (!M::kBf16 && top > 0.f)

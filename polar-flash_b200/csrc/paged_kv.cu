@@ -4,9 +4,10 @@
 //   (x[i], x[i + hd/2]) -> (x1 c - x2 s, x1 s + x2 c),
 // every product and sum rounded on its own as pf_rope_kv rounds them, then
 // the row is stored (16 or 32 bits) and, for keys and values, written into
-// its page, quantized by the formulas of pf_kv_quantize.  Bound by memory in
-// large calls (see launch_rope), by a chain of four dependent reads in small
-// ones (cu_seqlens, the lengths, the table, the row: 2.8 us for 64 tokens).
+// its page, quantized by the formulas of pf_kv_quantize.  Large calls are bound
+// by memory where rows are 16 bits wide, by instructions where they are
+// quantized (see launch_rope); small ones by a chain of four dependent reads
+// (cu_seqlens, the lengths, the table, the row: 2.8 us for 64 tokens).
 #include <math.h>
 
 #include "common.cuh"
@@ -214,8 +215,9 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kv_kernel(const RopeA
 // Four rows per warp where the rows fill the machine more than once, one where
 // the call is short of warps.  48 rows of 128 per token into int8 pages, one
 // and four rows per warp: 64 tokens 3.7 and 5.0 us, 256 5.8 and 6.1, 700 11.5
-// and 10.2, 8000 99.5 and 73.7 (bound by memory: 340 MB, 52 us at the copy rate;
-// bf16 pages 62 us).
+// and 10.2, 8000 99.5 and 73.7.  Of that call the bytes are 49 us at the copy rate,
+// and the same into bf16 pages, 332 MB for 316, takes 62 us: what bounds it is
+// its instructions, 168 a row, 0.79 issued a cycle and scheduler.
 template <int HD, int MODE, typename TI, typename TO>
 cudaError_t launch_rope(const RopeArgs& a, cudaStream_t s) {
   const long long rows = a.nh + 2 * a.pages.nkv, warps = kRopeThreads / 32;

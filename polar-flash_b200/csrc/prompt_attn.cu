@@ -34,9 +34,13 @@
 // over 1800 (reads 45, maximum 330, exponentials 1300, P 150), 100 until the
 // products are issued, 1370 for P V and the next scores; the other tile's chain
 // fills half of that.  The exponentials (16384 a tile, 16 a cycle and SM) are
-// the longest part.  8192 tokens, 32 heads over 8, bf16: 443 us in a burst of
-// three calls (1.24 PFLOP/s), 515 us sustained under the power limit.  Tried and
-// slower there.  Sustained, each beside the form of its day: two threads per row
+// the longest part.  8192 tokens, 32 heads over 8, bf16: 440 us in a burst of
+// three calls (1.25 PFLOP/s), 515 us sustained under the power limit.  Heads of
+// 96 take the form of 128 (12 prompts to 1500 tokens, 52 and 51 us), 40 that of
+// 64 (45 and 42): the softmax, which costs the same, bounds them.  Weights are
+// rounded to 16 bits because that is what the products take beside a 16-bit v;
+// it adds as much again as the output's own rounding (2.0e-3 normwise against
+// 1.6e-3 in bf16).  Tried and slower there.  Sustained, each beside the form of its day: two threads per row
 // (595 against 545 us), three pairs of exponentials in eight on the FMA pipes
 // instead of one (527 against 516).  In bursts, against 443 us: steps of 64 keys
 // with two S buffers (558: 64-wide score products wait for Q's reads from shared

@@ -53,7 +53,7 @@ class BatchDecoder:
     "2bit_asym").  A prompt's own attention runs in `prompt_dtype` (fp16 or bf16)
     on its keys and values as they are; later tokens read them from the cache, as
     it holds them.  head_dim is 64 or 128.  Calls on one decoder stay on one
-    stream."""
+    stream of its device, which is the current one."""
 
     def __init__(self, config: Dict, layers: List[DecoderLayer], embed: torch.Tensor, final_norm: torch.Tensor,
                  lm_head: torch.Tensor, max_seqs: int, max_seq: int, num_pages: int, page_size: int = 64,

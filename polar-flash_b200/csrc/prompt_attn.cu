@@ -39,12 +39,14 @@
 // 96 take the form of 128 (12 prompts to 1500 tokens, 52 and 51 us), 40 that of
 // 64 (45 and 42): the softmax, which costs the same, bounds them.  Weights are
 // rounded to 16 bits because that is what the products take beside a 16-bit v;
-// it adds as much again as the output's own rounding (2.0e-3 normwise against
-// 1.6e-3 in bf16).  Tried and slower there.  Sustained, each beside the form of its day: two threads per row
-// (595 against 545 us), three pairs of exponentials in eight on the FMA pipes
+// it takes the normwise error in bf16 from the 1.6e-3 of the output's own
+// rounding to 2.0e-3.
+// Tried and slower.  Sustained, each beside the form of its day: two threads per
+// row (595 against 545 us), three pairs of exponentials in eight on the FMA pipes
 // instead of one (527 against 516).  In bursts, against 443 us: steps of 64 keys
 // with two S buffers (558: 64-wide score products wait for Q's reads from shared
-// memory), a warp of products per tile (534: their products interleave).
+// memory), a warp of products per tile (534: their products interleave), and a
+// warp that waits together and votes (457).
 // Every wait is bounded.  One that gives up raises the CTA's abort flag, on
 // which the other waits give up too; the status word is marked, and rows that
 // were still waiting become NaN.  The warps then meet at a barrier, and only
@@ -435,8 +437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           commit(sbar + 8 * t);
         };
-        // The steps of one thread: it waits and issues by itself (a vote of the warp at each wait took 3 % of the
-        // kernel).  The warp meets before the last step, where a V tile that the sequence does not fill needs
+        // The steps are one thread's: it waits and issues by itself (with a vote of the warp at each wait 8192 tokens
+        // took 457 us for 445).  The warp meets before the last step, where a V tile that the sequence does not fill needs
         // zeros, and once more at the end; `ok` is the same in all lanes there.
         bool ok = true;
         for (int from = 0; ok && from < most;) {
